@@ -5,13 +5,14 @@
 :class:`ExpertLayer` holds a router and gated experts, ``y = sum_j w_j
 (silu(x G_e) * (x U_e)) D_e`` over a token's top_k experts e. ``serve`` computes
 it with the activation fused into the first product, in 16 bits or with 8-bit
-weights and activations; ``train`` gives torch's autograd the router, the products
+weights and activations, from the parameters as they are; ``train`` gives torch's autograd the router, the products
 and the weighted sum with their gradients. The program serves a decoding step and a
 prompt, trains a few steps, and prints what each took.
 """
 from __future__ import annotations
 
 import argparse
+import weakref
 
 import torch
 
@@ -132,7 +133,6 @@ class ExpertLayer:
         self.router = made(width, experts, dt=torch.float32)
         self.up = made(experts, width, 2 * hidden)
         self.down = made(experts, hidden, width)
-        self._f8 = None
 
     def parameters(self):
         return [self.router, self.up, self.down]
@@ -146,30 +146,43 @@ class ExpertLayer:
         y = _Product.apply(torch.nn.functional.silu(gate) * u, self.down, routing, False)
         return _Combine.apply(y, weights, routing)
 
-    def quantize(self) -> None:
-        """The experts' weights in 8 bits, rows of the output contiguous: once."""
-        out = []
-        for w in (self.up, self.down):
+    def quantize(self, out: list | None = None) -> list:
+        """The experts' weights as they are, in 8 bits, rows of the output contiguous:
+        up, its scales, down, its scales. `out`: what an earlier call gave, written
+        again."""
+        made = []
+        for i, w in enumerate((self.up, self.down)):
             w = w.transpose(1, 2).contiguous()
             e, n, k = w.shape
-            q = torch.empty(w.shape, dtype=torch.float8_e4m3fn, device=w.device)
-            s = torch.empty((e, -(-n // 128), -(-k // 128)), device=w.device)
+            q, s = out[2 * i:2 * i + 2] if out else (
+                torch.empty(w.shape, dtype=torch.float8_e4m3fn, device=w.device),
+                torch.empty((e, -(-n // 128), -(-k // 128)), device=w.device))
             tb.quantize_f8(w, q, s, block_rows=128)
-            out += [q, s]
-        self._f8 = out
+            made += [q, s]
+        return made
 
     def server(self, tokens: int, f8: bool = False) -> "Server":
         return Server(self, tokens, f8)
 
 
+def _state(w):
+    """What tells a parameter's values apart: the tensor and its count of changes
+    (None: inference tensors have none)."""
+    return weakref.ref(w), None if w.is_inference() else w._version
+
+
 class Server:
-    """Descriptors and buffers for batches of `tokens` tokens; `run` is the layer."""
+    """Descriptors and buffers for batches of `tokens` tokens; `run` is the layer.
+
+    `f8`: the server holds the weights in 8 bits, and `run` makes them again, in
+    place, when a parameter was replaced or changed. Of changes through `.data` or
+    other libraries' pointers torch counts no version: `refresh` says that there
+    were some. Inference tensors have no version at all: from those every `run`
+    makes the weights again."""
 
     def __init__(self, layer: ExpertLayer, tokens: int, f8: bool):
         dev, code = layer.up.device, DTYPES[layer.dtype]
-        self.layer, self.f8 = layer, f8
-        if f8 and layer._f8 is None:
-            layer.quantize()
+        self.layer, self.f8, self.weights = layer, f8, None
         slots = tokens * layer.top_k
         self.routing = Routing(tokens, layer.experts, layer.top_k, dev)
         self.h = torch.empty((slots, layer.hidden), dtype=layer.dtype, device=dev)
@@ -187,12 +200,26 @@ class Server:
                         torch.empty((rows, -(-cols // 128)), device=dev))
 
             self.xq, self.hq = e4m3(tokens, layer.width), e4m3(slots, layer.hidden)
+            self.refresh()
+
+    def refresh(self) -> None:
+        """The parameters as they are now, in 8 bits (16-bit servers read them anyway)."""
+        if not self.f8:
+            return
+        self.weights = self.layer.quantize(self.weights)
+        self._of = [_state(w) for w in (self.layer.up, self.layer.down)]
+
+    def _changed(self) -> bool:
+        return any(ref() is not w or version is None or version != w._version
+                   for w, (ref, version) in zip((self.layer.up, self.layer.down), self._of))
 
     def run(self, x):
         layer, r = self.layer, self.routing
         r.run(x.float() @ layer.router)
         if self.f8:
-            up, up_scale, down, down_scale = layer._f8
+            if self._changed():
+                self.refresh()
+            up, up_scale, down, down_scale = self.weights
             tb.quantize_f8(x, *self.xq)
             self.first.launch(self.xq[0], up, self.h, offsets=r.offsets, rows=r.rows,
                               a_scale=self.xq[1], b_scale=up_scale)
