@@ -12,6 +12,7 @@ prompt, trains a few steps, and prints what each took.
 from __future__ import annotations
 
 import argparse
+import functools
 import weakref
 
 import torch
@@ -39,6 +40,37 @@ class Routing:
                  workspace=self.workspace)
 
 
+class _Once(torch.autograd.Function):
+    """The first `n` tensors, gradients made of the others: to go back through them raises."""
+
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tuple(t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the gradients of an expert layer cannot be differentiated again")
+
+
+def _once(backward):
+    """A backward pass of kernels that autograd sees nothing of. Where its gradients get
+    a graph of their own (create_graph), that graph ends in an error at all they were
+    made of; torch's once_differentiable lets them pass as constants where the
+    incoming gradient is one, and where no leaf that is asked for lies behind it."""
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        at = [i for i, g in enumerate(out) if g is not None]
+        tied = _Once.apply(len(at), *(out[i] for i in at), *ctx.saved_tensors, *grads)
+        return tuple(tied[at.index(i)] if i in at else None for i in range(len(out)))
+
+    return run
+
+
 class _Route(torch.autograd.Function):
     """logits -> weights, and the routing's order in `routing`."""
 
@@ -50,6 +82,7 @@ class _Route(torch.autograd.Function):
         return routing.weights
 
     @staticmethod
+    @_once
     def backward(ctx, dweights):
         (logits,) = ctx.saved_tensors
         dlogits = torch.empty_like(logits)
@@ -76,6 +109,7 @@ class _Product(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_once
     def backward(ctx, dy):
         x, w = ctx.saved_tensors
         groups, k, n = w.shape
@@ -108,6 +142,7 @@ class _Combine(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_once
     def backward(ctx, dout):
         y, weights = ctx.saved_tensors
         dy, dw = torch.zeros_like(y), torch.empty_like(weights)

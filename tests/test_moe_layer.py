@@ -167,3 +167,38 @@ def test_8_bit_weights_of_changes_that_no_version_counts(log):
         server = layer.server(9, f8=True)
         layer.up.mul_(-1.5)
         assert _near(server.run(x), layer.server(9).run(x))
+
+
+def _train(layer, x, trained=("router", "up", "down")):
+    for name in trained:
+        setattr(layer, name, getattr(layer, name).detach().requires_grad_(True))
+    return layer.train(x)
+
+
+@pytest.mark.parametrize("trained", [("router",), ("up",), ("down",), ("router", "up", "down")])
+@pytest.mark.parametrize("loss", [lambda out: out.float().sum(),
+                                  lambda out: out.float().square().sum()])
+def test_a_second_derivative_raises(log, trained, loss):
+    """The gradients come from kernels that autograd sees nothing of: to differentiate
+    them again is an error, not a term of zero, also beside terms that it does see and
+    where the loss is linear, so that the output's gradient is a constant."""
+    layer = _layer()
+    out = _train(layer, _x(layer), trained)
+    params = [getattr(layer, name) for name in trained]
+    grads = torch.autograd.grad(loss(out), params, create_graph=True)
+    penalty = sum(g.float().square().sum() for g in grads)
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        torch.autograd.grad(penalty + loss(out), params, retain_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        penalty.backward()
+
+
+def test_first_derivatives_with_a_graph_are_the_same(log):
+    """Of the parameters whose gradients do not pass torch's silu, which has a
+    formula of its own for gradients with a graph."""
+    layer = _layer()
+    out = _train(layer, _x(layer))
+    params = [layer.router, layer.down]
+    plain = torch.autograd.grad(out.float().sum(), params, retain_graph=True)
+    graph = torch.autograd.grad(out.float().sum(), params, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, graph))
