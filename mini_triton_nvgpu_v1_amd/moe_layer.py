@@ -5,9 +5,10 @@
 :class:`ExpertLayer` holds a router and gated experts, ``y = sum_j w_j
 (silu(x G_e) * (x U_e)) D_e`` over a token's top_k experts e. ``serve`` computes
 it with the activation fused into the first product, in 16 bits or with 8-bit
-weights and activations, from the parameters as they are; ``train`` gives torch's autograd the router, the products
-and the weighted sum with their gradients. The program serves a decoding step and a
-prompt, trains a few steps, and prints what each took.
+weights and activations, from the parameters as they are; ``train`` gives
+torch's autograd the router, the products and the weighted sum with their
+gradients. The program serves a decoding step and a prompt, trains a few steps,
+and prints what each took.
 """
 from __future__ import annotations
 
@@ -23,20 +24,20 @@ DTYPES = {torch.float16: tb.DTYPE_F16, torch.bfloat16: tb.DTYPE_BF16}
 
 
 class Routing:
-    """The buffers of one batch's routing."""
+    """The buffers of one batch's routing; the weights are the caller's (in training
+    they are an output that autograd's node holds on to, and that node the routing)."""
 
     def __init__(self, tokens: int, experts: int, top_k: int, device):
         i32 = torch.int32
         self.ids = torch.empty((tokens, top_k), dtype=i32, device=device)
-        self.weights = torch.empty((tokens, top_k), device=device)
         self.slots = torch.empty((tokens, top_k), dtype=i32, device=device)
         self.rows = torch.empty(tokens * top_k, dtype=i32, device=device)
         self.offsets = torch.empty(experts + 1, dtype=i32, device=device)
         size = tb.route_workspace_bytes(tokens, experts, top_k)
         self.workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
-    def run(self, logits) -> None:
-        tb.route(logits, self.ids, self.weights, self.slots, self.rows, self.offsets,
+    def run(self, logits, weights) -> None:
+        tb.route(logits, self.ids, weights, self.slots, self.rows, self.offsets,
                  workspace=self.workspace)
 
 
@@ -76,17 +77,18 @@ class _Route(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, routing):
-        routing.run(logits)
+        weights = torch.empty(routing.ids.shape, device=logits.device)
+        routing.run(logits, weights)
         ctx.save_for_backward(logits)
-        ctx.routing = routing
-        return routing.weights
+        ctx.ids = routing.ids
+        return weights
 
     @staticmethod
     @_once
     def backward(ctx, dweights):
         (logits,) = ctx.saved_tensors
         dlogits = torch.empty_like(logits)
-        tb.route_backward(dweights.contiguous(), logits, ctx.routing.ids, dlogits)
+        tb.route_backward(dweights.contiguous(), logits, ctx.ids, dlogits)
         return dlogits, None
 
 
@@ -220,6 +222,7 @@ class Server:
         self.layer, self.f8, self.weights = layer, f8, None
         slots = tokens * layer.top_k
         self.routing = Routing(tokens, layer.experts, layer.top_k, dev)
+        self.route_weights = torch.empty((tokens, layer.top_k), device=dev)
         self.h = torch.empty((slots, layer.hidden), dtype=layer.dtype, device=dev)
         # slots without a pair are read by no token
         self.y = torch.empty((slots, layer.width), dtype=layer.dtype, device=dev)
@@ -250,7 +253,7 @@ class Server:
 
     def run(self, x):
         layer, r = self.layer, self.routing
-        r.run(x.float() @ layer.router)
+        r.run(x.float() @ layer.router, self.route_weights)
         if self.f8:
             if self._changed():
                 self.refresh()
@@ -264,7 +267,7 @@ class Server:
         else:
             self.first.launch(x, layer.up, self.h, offsets=r.offsets, rows=r.rows)
             self.second.launch(self.h, layer.down, self.y, offsets=r.offsets)
-        tb.combine(self.y, r.slots, self.out, weights=r.weights)
+        tb.combine(self.y, r.slots, self.out, weights=self.route_weights)
         return self.out
 
 

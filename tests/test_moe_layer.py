@@ -1,6 +1,8 @@
 """What the example layer keeps, for how long, and what autograd sees of it: its own
 classes on the CPU, over operators that stand in for the kernels. Like the kernels
 they write the caller's buffers behind autograd's back (`.data`: no version counts)."""
+import gc
+import weakref
 from types import SimpleNamespace
 
 import pytest
@@ -202,3 +204,31 @@ def test_first_derivatives_with_a_graph_are_the_same(log):
     plain = torch.autograd.grad(out.float().sum(), params, retain_graph=True)
     graph = torch.autograd.grad(out.float().sum(), params, create_graph=True)
     assert all(torch.equal(a, b) for a, b in zip(plain, graph))
+
+
+@pytest.mark.parametrize("backward", [True, False])
+def test_a_step_leaves_nothing_behind(log, monkeypatch, backward):
+    """A step's routing and its buffers are freed with the step's graph, without
+    Python's cycle collector."""
+    alive = []
+
+    class Routing(moe_layer.Routing):
+        def __init__(self, *args):
+            super().__init__(*args)
+            alive.append(weakref.ref(self))
+            alive.extend(weakref.ref(t) for t in vars(self).values()
+                         if isinstance(t, torch.Tensor))
+
+    monkeypatch.setattr(moe_layer, "Routing", Routing)
+    layer = _layer()
+    gc.collect()
+    gc.disable()
+    try:
+        out = _train(layer, _x(layer))
+        if backward:
+            out.float().sum().backward()
+        assert len(alive) > 4 and alive[0]() is not None
+        del out
+        assert [r for r in alive if r() is not None] == []
+    finally:
+        gc.enable()
