@@ -117,18 +117,20 @@ class _Product(torch.autograd.Function):
         groups, k, n = w.shape
         code, r = DTYPES[x.dtype], ctx.routing
         dy = dy.contiguous()
-        # of the rows: the product with the transposed weights, slot by slot
-        drows = torch.zeros((dy.shape[0], k), dtype=x.dtype, device=x.device)
-        tb.GroupedDesc.from_config(groups=groups, n=k, k=n, dtype=code, c_dtype=code,
-                                   b_layout=tb.B_NK).launch(dy, w, drows, offsets=r.offsets)
-        dw = torch.empty_like(w)
-        tb.GroupedDesc.from_config(kind=tb.GROUPED_WGRAD, groups=groups, n=n, k=k, dtype=code,
-                                   c_dtype=code).launch(
-            x, dy, dw, offsets=r.offsets, rows=r.rows if ctx.gather else None)
-        if not ctx.gather:
-            return drows, dw, None, None
-        dx = torch.empty_like(x)  # a token's rows, each with weight one
-        tb.combine(drows, r.slots, dx)
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            # of the rows: the product with the transposed weights, slot by slot
+            dx = torch.zeros((dy.shape[0], k), dtype=x.dtype, device=x.device)
+            tb.GroupedDesc.from_config(groups=groups, n=k, k=n, dtype=code, c_dtype=code,
+                                       b_layout=tb.B_NK).launch(dy, w, dx, offsets=r.offsets)
+            if ctx.gather:
+                drows, dx = dx, torch.empty_like(x)  # a token's rows, each with weight one
+                tb.combine(drows, r.slots, dx)
+        if ctx.needs_input_grad[1]:
+            dw = torch.empty_like(w)
+            tb.GroupedDesc.from_config(kind=tb.GROUPED_WGRAD, groups=groups, n=n, k=k,
+                                       dtype=code, c_dtype=code).launch(
+                x, dy, dw, offsets=r.offsets, rows=r.rows if ctx.gather else None)
         return dx, dw, None, None
 
 
@@ -147,9 +149,10 @@ class _Combine(torch.autograd.Function):
     @_once
     def backward(ctx, dout):
         y, weights = ctx.saved_tensors
-        dy, dw = torch.zeros_like(y), torch.empty_like(weights)
+        dy = torch.zeros_like(y)
+        dw = torch.empty_like(weights) if ctx.needs_input_grad[1] else None
         tb.combine_backward(dout.contiguous(), y, ctx.routing.slots, weights, dy, dw)
-        return dy, dw, None
+        return dy if ctx.needs_input_grad[0] else None, dw, None
 
 
 class ExpertLayer:

@@ -232,3 +232,28 @@ def test_a_step_leaves_nothing_behind(log, monkeypatch, backward):
         assert [r for r in alive if r() is not None] == []
     finally:
         gc.enable()
+
+
+@pytest.mark.parametrize("trained, want", [
+    (("x",), ["route_backward", "combine_backward", "dweights", "rows", "rows", "combine"]),
+    (("router",), ["route_backward", "combine_backward", "dweights"]),
+    (("up",), ["combine_backward", "rows", "wgrad"]),
+    (("down",), ["combine_backward", "wgrad"]),
+    (("x", "router", "up", "down"), ["route_backward", "combine_backward", "dweights", "rows",
+                                     "rows", "wgrad", "wgrad", "combine"])])
+def test_only_the_gradients_asked_for_are_computed(log, trained, want):
+    layer = _layer()
+    leaves = {"x": _x(layer), "router": layer.router, "up": layer.up, "down": layer.down}
+    for name in trained:
+        leaves[name].requires_grad_(True)
+    all_of = _layer()
+    every = {"x": _x(layer), "router": all_of.router, "up": all_of.up, "down": all_of.down}
+    for t in every.values():
+        t.requires_grad_(True)
+    all_of.train(every["x"]).float().sum().backward()
+    out = layer.train(leaves["x"])
+    log.clear()
+    out.float().sum().backward()
+    assert sorted(log) == sorted(want)
+    for name in trained:
+        assert torch.equal(leaves[name].grad, every[name].grad)
