@@ -115,7 +115,7 @@ struct GroupedTile {
   static constexpr int slot_mid(int o) { return spread_slot(S0_MID, o); }
   static constexpr int slot_last(int o) { return spread_slot(S0_LAST, o); }
   static constexpr int NSLOT = KS * NM;
-    static constexpr int SPREAD = STAGES == 2 ? NSLOT * 5 / 8 : NSLOT - NSLOT / 8;
+  static constexpr int SPREAD = STAGES == 2 ? NSLOT * 5 / 8 : NSLOT - NSLOT / 8;
   static constexpr int load_slot(int l) { return l * SPREAD / LPT; }
   static constexpr int PER_SLOT = 3;
   static constexpr int mid_op(int m, int k) {

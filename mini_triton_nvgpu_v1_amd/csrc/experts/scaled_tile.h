@@ -66,6 +66,7 @@ struct ScaledTile {
   static constexpr int E_ROWB = WTN * 4, EPI_REGION = 16 * E_ROWB;
   // refill load l goes body slot load_slot(l): slots from the barrier on
   static constexpr int load_slot(int l) { return l * (NM * 3 / 8) / LPT; }
+  static_assert(load_slot(LPT - 1) < NM, "a k-tile's loads are issued before the next barrier");
   static_assert(TI % 4 == 0 && WTN % 32 == 0, "pairs of rows, two buffers of them");
   static_assert(LA * NT * 16 == A_BYTES && LB * NT * 16 == B_BYTES, "whole load rounds");
   static_assert(RPR % 32 == 0, "rounds of whole swizzle periods and column pairs");
@@ -157,9 +158,12 @@ __device__ __forceinline__ void scaled_tile(const GroupedParams &p, const TilePl
     *(TBK_LDS uint32_t *)(uintptr_t)(lds0 + G::TABLE + t * 4u) = v;
   }
   // Step x: in phase x % 4, units x % 4 and x % 4 + 4 of k-tiles 4 (x / 4) .. + 3, a
-  // wave each. The steps of a group of four k-tiles end two barriers before its
-  // first k-tile is read (three with three stages), and the group whose place it
-  // takes has been read by then.
+  // wave each. The last step of a group of four k-tiles, 4 g + 3, is the last load of
+  // k-tile 4 g: issued before the barrier that ends the wait for that k-tile (the
+  // static_assert on its slot), waited for with it and read right behind. So
+  // STAGES - 1 barriers lie between, one with two stages: no step may come later.
+  // The group whose place the first step takes was read before the barrier that this
+  // step is issued behind.
   auto load_scales = [&](int x) {
     const int u = x % 4 + (wave / 4) * 4, kt = (x & ~3) + wave % 4;
     const bool live = u < G::UNITS && kt < nk;
