@@ -381,7 +381,8 @@ typedef struct tb_grouped_desc tb_grouped_desc;
  * group's B or C_e spans less than 2 GiB. */
 int tb_grouped_create(const tb_grouped_config *cfg, tb_grouped_desc **out);
 int tb_grouped_get_config(const tb_grouped_desc *desc, tb_grouped_config *out);
-/* Bytes of workspace that a launch over `slots` slots needs (0: none). */
+/* Bytes of workspace that a launch over `slots` slots needs (0: none). No
+ * build of today needs any. */
 size_t tb_grouped_workspace_bytes(const tb_grouped_desc *desc, int64_t slots);
 /* offsets: groups + 1 (NULL with one group: all slots); rows: slots, or NULL
  * where slot i is row i of A. A slot whose row lies outside A counts as zeros

@@ -9,8 +9,8 @@
 // weights are the same for all its lanes. The rows on their way are held as
 // they lie in memory and become f32 when they are added: half the registers,
 // six waves on a SIMD unit rather than four in the gradient.
-// 8192 tokens of 8 bf16 rows of 4096: the sum takes 101 us (6.0 TB/s), its
-// gradients 232 us (4.9 TB/s read and written; 269 us with rows held as f32).
+// 8192 tokens of 8 bf16 rows of 4096: the sum takes 101-104 us (5.8-6.0 TB/s),
+// its gradients 229-232 us (4.9 TB/s read and written; 269 us with rows held as f32).
 #include "experts_device.h"
 
 namespace tbk {

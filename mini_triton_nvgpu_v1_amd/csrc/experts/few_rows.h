@@ -11,9 +11,9 @@
 //    (block l / 16 of 4): 32 x 128 of the weights in 8 loads of 4 whole
 //    256-byte pieces. One byte permute per register turns the 8 x 8 values that
 //    a lane holds into 8 fragments, column 8 (l % 16) + j for the j-th.
-// One token's 8 of 128 experts, 4096 x 2048 bf16 n x k: 28 us, 4.8 TB/s of weights
-// (64 workgroups of 128 x 128 tiles 54 us); 13 tokens, 6 of 64, 2048 x 2048 f16 k x
-// n: 62 us, 6.3 TB/s with the last-level cache; e4m3, 16 x 8192 x 4096: 13 us, four
+// One token's 8 of 128 experts, 4096 x 2048 bf16 n x k: 28-30 us, 4.5-4.8 TB/s of
+// weights (64 workgroups of 128 x 128 tiles 54 us); 13 tokens, 6 of 64, 2048 x 2048 f16 k x
+// n: 62-68 us, 5.7-6.3 TB/s with the last-level cache; e4m3, 16 x 8192 x 4096: 13 us, four
 // chunks a wave, so latency.
 // Rows of A that a tile lacks read nothing. Products and sums are f32 (e4m3: the
 // instruction's own sums within a block, scaled_tile.h says how exact); the

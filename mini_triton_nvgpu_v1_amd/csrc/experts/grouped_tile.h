@@ -757,7 +757,8 @@ __global__ __launch_bounds__(WGM *WGN * 64, 1) void grouped_wgrad(GroupedParams 
   // The groups' depths differ, so every XCD (blocks go round them) takes an eighth
   // of each group's tiles rather than whole groups: 8192 tokens of 2 of 16 experts,
   // C 4096 x 2048 in f32, 361 us against 408 with whole groups (with later steps
-  // 298: 922 TFLOP/s, and 537 MB of C written after the products).
+  // 298-310 at its fastest and 323-339 on average: 811-922 TFLOP/s, and 537 MB of C
+  // written after the products).
   const int per = tiles_m * tiles_n, per_xcd = (per + 7) / 8;
   const int i = blockIdx.x / 8, group = i / per_xcd;
   const int w = (int)(blockIdx.x % 8) * per_xcd + i % per_xcd;

@@ -23,10 +23,12 @@
 // refilled two k-tiles ahead, and the next k-tile's first pair and B's
 // fragments, each after its last use, are read.
 //
-// 8192 x 8192 x 4096 on 256 x 256 tiles: 256 us, 2.15 PFLOP/s. At 265 us it took 180
+// 8192 x 8192 x 4096 on 256 x 256 tiles: 256-268 us, 2.05-2.15 PFLOP/s. At 265 us it took 180
 // with the MFMAs alone (3.05 PFLOP/s, the clock the power allows), 238 without the
 // loads, 252 without the scaling: no one of them bounds it, they share a compute
-// unit whose 8 waves meet at a barrier every 128 of the depth. Three stages on 256 x
+// unit whose 8 waves meet at a barrier every 128 of the depth. By count LDS is a
+// bound of the same size as the matrix unit: a k-tile's 192 KB of fragment reads and
+// 64 KB of loads are 2048 clocks at 128 bytes each, its MFMAs 2048 clocks too. Three stages on 256 x
 // 128 tiles took 328 us, four on 128 x 128 463: the loads are not late.
 #pragma once
 
