@@ -201,7 +201,7 @@ class ExpertLayer:
             made += [q, s]
         return made
 
-    def server(self, tokens: int, f8: bool = False) -> "Server":
+    def server(self, tokens: int, f8: bool | list = False) -> "Server":
         return Server(self, tokens, f8)
 
 
@@ -218,11 +218,14 @@ class Server:
     place, when a parameter was replaced or changed. Of changes through `.data` or
     other libraries' pointers torch counts no version: `refresh` says that there
     were some. Inference tensors have no version at all: from those every `run`
-    makes the weights again."""
+    makes the weights again. Weights that the caller quantized, `f8` what
+    ExpertLayer.quantize gave, can be shared by servers and stay as they are until
+    it is given them again."""
 
-    def __init__(self, layer: ExpertLayer, tokens: int, f8: bool):
+    def __init__(self, layer: ExpertLayer, tokens: int, f8: bool | list):
         dev, code = layer.up.device, DTYPES[layer.dtype]
-        self.layer, self.f8, self.weights = layer, f8, None
+        self.layer, self.f8 = layer, bool(f8)
+        self.weights, self._of = (f8, None) if isinstance(f8, list) else (None, ())
         slots = tokens * layer.top_k
         self.routing = Routing(tokens, layer.experts, layer.top_k, dev)
         self.route_weights = torch.empty((tokens, layer.top_k), device=dev)
@@ -241,18 +244,21 @@ class Server:
                         torch.empty((rows, -(-cols // 128)), device=dev))
 
             self.xq, self.hq = e4m3(tokens, layer.width), e4m3(slots, layer.hidden)
-            self.refresh()
+            if self.weights is None:
+                self.refresh()
 
     def refresh(self) -> None:
         """The parameters as they are now, in 8 bits (16-bit servers read them anyway)."""
         if not self.f8:
             return
         self.weights = self.layer.quantize(self.weights)
-        self._of = [_state(w) for w in (self.layer.up, self.layer.down)]
+        if self._of is not None:
+            self._of = [_state(w) for w in (self.layer.up, self.layer.down)]
 
     def _changed(self) -> bool:
-        return any(ref() is not w or version is None or version != w._version
-                   for w, (ref, version) in zip((self.layer.up, self.layer.down), self._of))
+        return self._of is not None and any(
+            ref() is not w or version is None or version != w._version
+            for w, (ref, version) in zip((self.layer.up, self.layer.down), self._of))
 
     def run(self, x):
         layer, r = self.layer, self.routing
@@ -294,9 +300,10 @@ def main() -> None:
     layer = ExpertLayer(width=2048, hidden=1024, experts=64, top_k=6)
     g = torch.Generator(device="cuda")
     g.manual_seed(1)
+    weights8 = layer.quantize()
     for tokens in (13, args.tokens):
         x = torch.randn((tokens, layer.width), generator=g, device="cuda").to(layer.dtype)
-        plain, f8 = layer.server(tokens), layer.server(tokens, f8=True)
+        plain, f8 = layer.server(tokens), layer.server(tokens, f8=weights8)
         a, b = plain.run(x).float(), f8.run(x).float()
         off = float((a - b).norm() / a.norm())
         print(f"serving {tokens} tokens: {_us(lambda: plain.run(x)):.0f} us in 16 bits, "

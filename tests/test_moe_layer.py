@@ -257,3 +257,21 @@ def test_only_the_gradients_asked_for_are_computed(log, trained, want):
     assert sorted(log) == sorted(want)
     for name in trained:
         assert torch.equal(leaves[name].grad, every[name].grad)
+
+
+def test_8_bit_weights_that_the_caller_keeps(log):
+    """Weights that the caller quantized are shared by servers, also of inference
+    tensors, and made again when the caller says so."""
+    with torch.inference_mode():
+        layer = _layer()
+        weights = layer.quantize()
+        servers = [layer.server(n, f8=weights) for n in (9, 5)]
+        for n, server in zip((9, 5), servers):
+            server.run(_x(layer, n))
+            assert all(a is b for a, b in zip(server.weights, weights))
+        assert log.count("weights to 8 bits") == 2
+        layer.up.mul_(-1.5)
+        layer.quantize(weights)
+        for n, server in zip((9, 5), servers):
+            assert _near(server.run(_x(layer, n)), layer.server(n).run(_x(layer, n)))
+        assert log.count("weights to 8 bits") == 4
